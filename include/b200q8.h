@@ -505,8 +505,8 @@ b200q8_status_t b200q8_kv_read(const b200q8_kv_cache * cache, const b200q8_kv_ba
  * q and out rows are n_head * head_dim values, type B200Q8_SRC_* for both;
  * scale 0 means 1/sqrt(head_dim).  Scores, softmax and sums are fp32; q and
  * the weights enter the tensor cores with 22 bits (as integer or fp16 parts)
- * and codes and scales exactly, so F32 results are as exact as plain fp32 ones
- * (bf16 rows: weights of 11 bits).  A weight is held to 2^-22 of itself or
+ * and codes and scales exactly, so F32 results are as exact as plain fp32 ones,
+ * and 16-bit ones such results rounded once.  A weight is held to 2^-22 of itself or
  * 2^-32 of the row's largest, whichever is more.  Cells a row does not see
  * never contribute, whatever they hold.  On a ring cache a window is required and
  * window + max_len - 1 may not pass n_ctx - sinks.  n_head / n_kv <= 64.

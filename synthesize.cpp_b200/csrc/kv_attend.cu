@@ -46,9 +46,8 @@ namespace b200q8 {
 namespace {
 
 // NB: the most blocks a head has (EXACT: all of them).  K4, V4: 4-bit codes.
-// PARTS (TALL): fp16 parts of q and of the weights; 1 for bf16 rows, whose
-// 8 bits one fp16 value holds, with weights rounded to fp16 (2^-11 against
-// the result's own 2^-8).
+// PARTS (TALL): fp16 parts of q; 1 for bf16 rows, whose 8 bits one fp16 value
+// holds.  Weights have two parts for every type.
 template <int NB, bool EXACT, bool K4, bool V4, bool TALL, int PARTS>
 __global__ void __launch_bounds__(128)
     kv_attend_kernel(const KvAttendArgs a, const int wr, const int n_split, const int n_stages, const int tc) {
@@ -401,12 +400,7 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
                         for (int h = 0; h < kHalf; ++h) {
                             uint32_t hi, lo;
-                            if (TALL && PARTS == 1) {
-                                hi = h2_bits(__floats2half2_rn(sc[n][2 * h] * da, sc[n][2 * h + 1] * db));
-                                lo = 0u;
-                            } else {
-                                split_half(sc[n][2 * h] * da, sc[n][2 * h + 1] * db, hi, lo);
-                            }
+                            split_half(sc[n][2 * h] * da, sc[n][2 * h + 1] * db, hi, lo);
                             if (TALL) {
                                 ahi[2 * u + h] = hi;
                                 alo[2 * u + h] = lo;
@@ -419,11 +413,11 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (grp == 0) {
-                            mma_f16_first(acc[e], TALL && PARTS == 2 ? alo : ahi, f[0][e], f[1][e]);
+                            mma_f16_first(acc[e], TALL ? alo : ahi, f[0][e], f[1][e]);
                         } else {
-                            mma_f16(acc[e], TALL && PARTS == 2 ? alo : ahi, f[0][e], f[1][e]);
+                            mma_f16(acc[e], TALL ? alo : ahi, f[0][e], f[1][e]);
                         }
-                        if (TALL && PARTS == 2) {
+                        if (TALL) {
                             mma_f16(acc[e], ahi, f[0][e], f[1][e]);
                         }
                     }

@@ -5,11 +5,12 @@
 // turned into fp16 operands once per 128 rows instead of once per warp.  Keys
 // and values (code * scale: 19 bits or fewer) are an fp16 value plus the fp16
 // value of what that leaves over, exactly; so are q and the weights, to 22
-// bits, with PARTS = 2 (F32 and F16 rows): a product is hi*hi + hi*lo + lo*hi,
-// good to 2^-21.  With PARTS = 1 (bf16 rows: 2^-8 themselves) q, which fits,
-// and the weights (2^-11) are one fp16 value.  Key scales of a tile and value
-// scales of a group of tiles are first multiplied by a power of two, so that
-// fp16's range costs no bits.
+// bits: a product is hi*hi + hi*lo + lo*hi, good to 2^-21.  With PARTS = 1
+// (bf16 rows) q is one fp16 value, which holds its 8 bits.  Weights have both
+// parts for every type: with one, a tenth of the results of bf16 prompts were
+// rounded the other way, and a row's bits went by its call's length.  Key
+// scales of a tile and value scales of a group of tiles are first multiplied by
+// a power of two, so that fp16's range costs no bits.
 //
 // Roles of the 16 warps, handing over through mbarriers: one warp fetches
 // 64-cell tiles of the cache by bulk copies and looks for what is seen of them
@@ -485,19 +486,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
                 const float p0 = exp2_approx(fmaf(__uint_as_float(s[j]), f, -ref));
                 const float p1 = exp2_approx(fmaf(__uint_as_float(s[j + 1]), f, -ref));
                 add += p0 + p1;
-                if (PARTS == 2) {
-                    split_half(p0, p1, hi[j / 2], lo[j / 2]);
-                } else {
-                    hi[j / 2] = h2_bits(__floats2half2_rn(p0, p1));
-                }
+                split_half(p0, p1, hi[j / 2], lo[j / 2]);
             }
             sum += add;
             tc_after();
             const uint32_t pa = lanes + kColS + (uint32_t) (b * 64 + side * 16);
             tc_st16(pa, hi);
-            if (PARTS == 2) {
-                tc_st16(pa + 32, lo);
-            }
+            tc_st16(pa + 32, lo);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             if (threadIdx.x == 0) {
                 h->new_group[b] = begin;
@@ -688,7 +683,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
                         const uint32_t pc = tmem + kColS + (uint32_t) (b * 64), v = kv0 + kvb * L::kTile + L::kKBytes;
                         uint32_t       add = begin ? 0u : 1u;
 #pragma unroll
-                        for (int x = 2 - PARTS; x < 3; ++x) {
+                        for (int x = 0; x < 3; ++x) {
                             const uint32_t pa = pc + (x == 0 ? 32u : 0u);
                             const uint32_t va = v + (x == 1 ? (uint32_t) L::kVPart : 0u);
 #pragma unroll
