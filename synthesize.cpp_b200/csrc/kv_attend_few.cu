@@ -13,11 +13,13 @@
 // in fp16, gives row (h, b) the values of all blocks; those of block b count.
 // Rows 8 .. 15 hold the weights' second fp16 parts (of q: the second byte).
 //
-// The reference of the weights moves only when a weight times a value scale
-// would pass 2^15 (it is set so that the largest is 2^8 and has 7 bits to
-// grow), so that products add up in the tensor cores' accumulators; they are
-// moved to plain fp32 sums every kFold steps, because the tensor cores cut
-// their sums off where fp32 addition rounds.
+// The reference of the weights moves only when the largest weight times the
+// largest value scale of a lane's cells would pass 2^15 (it is set so that
+// they give 2^8 and have 7 bits to grow), or a weight kMostWeight (the weights
+// of cells whose values are zero must not overflow either), so that products
+// add up in the tensor cores' accumulators; they are moved to plain fp32 sums
+// every kFold steps, because the tensor cores cut their sums off where fp32
+// addition rounds.
 //
 // 64 streams of 500 to 8100 positions (keys in 8 bits, values in 4; 519 MB):
 // 145 us, 3.6 TB/s; its copies alone take 85 us.  It is bound by instructions
@@ -29,8 +31,9 @@
 namespace b200q8 {
 namespace {
 
-constexpr int kFold = 8;
-constexpr int kBias = 0x4b400000;  // an integer sum on top of it is the bits of 1.5 * 2^23 + sum
+constexpr int   kFold       = 8;
+constexpr float kMostWeight = 1.2379400392853803e27f;  // 2^90: sums over 2^30 cells stay below 2^120
+constexpr int   kBias       = 0x4b400000;  // an integer sum on top of it is the bits of 1.5 * 2^23 + sum
 
 // REGS: 168 with four warps a CTA (three CTAs an SM), 128 with eight (two, so that a cluster of 16 finds room)
 template <int NB, bool EXACT, bool K4, bool V4, int REGS>
@@ -274,9 +277,9 @@ __global__ void __maxnreg__(REGS) kv_attend_few_kernel(const KvAttendArgs a, con
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
                 pw[x] = exp2_approx(fmaf(sc[x], unscale, -ref));
-                peak  = fmaxf(peak, fabsf(pw[x] * dv[x]));
+                peak  = fmaxf(peak, pw[x]);
             }
-            if (__any_sync(0xffffffffu, valid && (peak > 32768.0f || (ref == -INFINITY && seen)))) {
+            if (__any_sync(0xffffffffu, valid && (peak * top > 32768.0f || peak > kMostWeight || (ref == -INFINITY && seen)))) {
                 float m = -INFINITY;
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {

@@ -33,3 +33,55 @@ def test_bf16_rows_are_f32_results_rounded_once(kv, dev, bits_k, bits_v, nh, n_k
     want, mass, reach = R.attend(c, q, pos, [2, 0, 1], lens, 0)
     ok = rounded(got, want, mass, reach)
     assert ok.all(), float((~ok).double().mean())
+
+
+# --------------------------------------------------------------------------- scores and value scales set one by one
+
+
+def scored(kv, dev, n_kv, hd, n_ctx, scores, bits_k=8, bits_v=8, seed=5):
+    """(cache, first): one slot, whose cell j scores scores[j] (to fp16) with a query whose value 0 is first and with
+    any other values: keys hold a one there and zeros elsewhere."""
+    c = make(kv, dev, 1, n_ctx, n_kv, hd, bits_k, bits_v, seed=seed)
+    s = torch.as_tensor(scores, dtype=torch.float64, device=dev)
+    zero, one = (0x88, 1) if bits_k == 4 else (0, 1)
+    c.k_codes[:] = zero
+    c.k_codes[0, :, :len(s), 0] = torch.where(s < 0, zero - one, zero + one).to(c.k_codes.dtype)
+    c.k_scales[0, :, :len(s)] = s.abs()[None, :, None].half()
+    assert R.places(hd, 4)[0] == 0
+    return c, hd ** 0.5
+
+
+def single(kv, c, first, nh, p, dtype=F32, window=0):
+    """The row at position p, over the kernels' and the plain form's results: (got, want, mass, reach)."""
+    dev = c.k_codes.device
+    q = rows(dev, 1, nh, c.head_dim, dtype, seed=77)
+    q[:, :, 0] = first
+    got = kv.attend(c, q, i32(dev, p), window=window)
+    return (got, *R.attend(c, q, [p], [0], [1], window))
+
+
+# query heads, kv heads, head size, cells, position: four warps a CTA, eight (long caches of few heads), the same for
+# a size of three blocks, one of two, one of one; several steps a warp; then the general kernel's forms for single rows
+SINGLES = [(16, 8, 128, 512, 300), (4, 2, 128, 8192, 6100), (4, 2, 96, 8192, 6100), (4, 2, 64, 8192, 6100),
+           (16, 8, 64, 512, 300), (4, 4, 32, 512, 300), (128, 64, 128, 2048, 2000), (16, 2, 128, 512, 300),
+           (4, 2, 256, 512, 300)]
+
+
+@pytest.mark.parametrize("bits_k,bits_v", [(4, 4), (8, 8), (8, 4), (4, 8)])
+@pytest.mark.parametrize("nh,n_kv,hd,n_ctx,p", SINGLES)
+@pytest.mark.parametrize("above", [45.0, 80.0, 150.0])
+def test_a_zero_valued_cell_of_high_score(kv, dev, nh, n_kv, hd, n_ctx, p, bits_k, bits_v, above):
+    """A cell whose values are all zero (a sink) takes nearly all the weight, wherever it lies among the cells that
+    warps and CTAs share out, first values of zero or not: results are what the others' share leaves."""
+    g = torch.Generator().manual_seed(nh + hd)
+    for zeros in ([0], [45], [p], [p // 2], [p // 2, p // 2 + 33, p - 70], list(range(40)) + [p - 9]):
+        s = torch.randn(p + 1, generator=g)
+        s[zeros[-1]] = above
+        c, first = scored(kv, dev, n_kv, hd, n_ctx, s, bits_k, bits_v)
+        c.v_scales[0, :, zeros] = 0.0
+        got, want, mass, reach = single(kv, c, first, nh, p)
+        # weights times value scales of below 2^-32 of the largest weight and scale lose bits; a cell brings 127 at most
+        most = R.values_of(c.v_codes[0, :, :p + 1], c.v_scales[0, :, :p + 1], "v").abs().amax()
+        tol = R.tolerance(want, mass, reach, F32) + (p + 1) * 2.0 ** -32 * most
+        assert torch.isfinite(got).all(), zeros
+        assert ((got.double() - want).abs() <= tol).all(), zeros
