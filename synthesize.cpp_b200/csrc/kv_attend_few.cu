@@ -14,12 +14,13 @@
 // Rows 8 .. 15 hold the weights' second fp16 parts (of q: the second byte).
 //
 // The reference of the weights moves only when the largest weight times the
-// largest value scale of a lane's cells would pass 2^15 (it is set so that
-// they give 2^8 and have 7 bits to grow), or a weight kMostWeight (the weights
-// of cells whose values are zero must not overflow either), so that products
-// add up in the tensor cores' accumulators; they are moved to plain fp32 sums
-// every kFold steps, because the tensor cores cut their sums off where fp32
-// addition rounds.
+// largest value scale of a lane's cells would pass 2^15, or a weight
+// kMostWeight (the weights of cells whose values are zero must not overflow
+// either).  It is set so that the largest product of both is below 2^8, as far
+// as weights stay below 2^-kZero: 7 bits to grow, and a product's fp16 parts
+// hold it to 2^-22 of itself or 2^-32 of the largest.  So products add up in the tensor cores'
+// accumulators; they are moved to plain fp32 sums every kFold steps, because
+// the tensor cores cut their sums off where fp32 addition rounds.
 //
 // 64 streams of 500 to 8100 positions (keys in 8 bits, values in 4; 519 MB):
 // 145 us, 3.6 TB/s; its copies alone take 85 us.  It is bound by instructions
@@ -33,6 +34,7 @@ namespace {
 
 constexpr int   kFold       = 8;
 constexpr float kMostWeight = 1.2379400392853803e27f;  // 2^90: sums over 2^30 cells stay below 2^120
+constexpr int   kZero       = -73;     // log2 of what a value scale of zero counts as
 constexpr int   kBias       = 0x4b400000;  // an integer sum on top of it is the bits of 1.5 * 2^23 + sum
 
 // REGS: 168 with four warps a CTA (three CTAs an SM), 128 with eight (two, so that a cluster of 16 finds room)
@@ -283,14 +285,12 @@ __global__ void __maxnreg__(REGS) kv_attend_few_kernel(const KvAttendArgs a, con
                 float m = -INFINITY;
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
-                    m = fmaxf(m, sc[x] * unscale);
+                    const int e = max(kZero, (int) (__float_as_uint(fabsf(dv[x])) >> 23) - 127);
+                    m           = fmaxf(m, fmaf(sc[x], unscale, (float) e));
                 }
-                m   = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m   = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float e    = (float) max(-25, (int) (__float_as_uint(top) >> 23) - 127);
-                const float next = fmaxf(ref, m + e - 7.0f);
+                m                = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m                = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const float next = fmaxf(ref, m - 7.0f);
                 if (valid && next > -INFINITY) {
                     const float alpha = exp2_approx(ref - next);  // 0 before the first cell
                     ref               = next;

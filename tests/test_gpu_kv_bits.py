@@ -85,3 +85,23 @@ def test_a_zero_valued_cell_of_high_score(kv, dev, nh, n_kv, hd, n_ctx, p, bits_
         tol = R.tolerance(want, mass, reach, F32) + (p + 1) * 2.0 ** -32 * most
         assert torch.isfinite(got).all(), zeros
         assert ((got.double() - want).abs() <= tol).all(), zeros
+
+
+@pytest.mark.parametrize("nh,n_kv,hd,n_ctx,p", SINGLES[:7])
+def test_single_rows_hold_products_of_weight_and_value_scale(kv, dev, nh, n_kv, hd, n_ctx, p):
+    """Large value scales at negligible weights, or large weights at values of zero, cost the products that count no
+    bits, in one step of the kernel or in steps one after another."""
+    tiny = 177 * 2.0 ** -24  # with few bits to spare in fp16
+    for at in ([3], [40], [p - 3], [3, 40, p - 40]):
+        s = torch.zeros(p + 1)
+        s[at] = -40.0
+        c, first = scored(kv, dev, n_kv, hd, n_ctx, s)
+        c.v_scales[0] = tiny
+        c.v_scales[0, :, at] = 32768.0
+        got, want, mass, reach = single(kv, c, first, nh, p)
+        assert ((got.double() - want).abs() <= R.tolerance(want, mass, reach, F32)).all(), at
+        s[at] = 45.0  # 65 octaves above
+        c, first = scored(kv, dev, n_kv, hd, n_ctx, s)
+        c.v_scales[0, :, at] = 0.0
+        got, want, mass, reach = single(kv, c, first, nh, p)
+        assert ((got.double() - want).abs() <= R.tolerance(want, mass, reach, F32)).all(), at
