@@ -11,9 +11,11 @@
 // ones.  q is first scaled by a power of two per row so that its largest
 // value lies in [2^14, 2^15), and weights are taken relative to a running
 // reference  ref = max_j s_j + e - 14  with 2^e <= max dv < 2^(e+1)  (log2
-// units), so that w * dv is below 2^15: neither part loses bits to fp16's
-// range.  The sum of weights uses the same reference, so the result is their
-// plain quotient.
+// units; the score's maximum runs, the scales' is a step's own, because large
+// scales at small weights would cost all later steps bits), so that w * dv is
+// below 2^15 and held to 2^-22 of itself or 2^-38 of the largest weight times
+// the step's largest scale.  The sum of weights uses the same reference, so the
+// result is their plain quotient.
 //
 // Work split.  A CTA takes a tile of query rows (tokens x heads of one kv
 // head, token major) of one run; a cluster of CTAs splits the tile's visible
@@ -327,7 +329,7 @@ __global__ void __launch_bounds__(128)
                 dmax = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, 1));
                 dmax = fmaxf(dmax, __shfl_xor_sync(0xffffffffu, dmax, 2));
             }
-            const int e_new = max(ref_e, (int) (__float_as_uint(dmax) >> 23) - 127);
+            const int e_new = max(-25, (int) (__float_as_uint(dmax) >> 23) - 127);
 
             // ---- weights relative to the new reference
             float alpha[kHalf];

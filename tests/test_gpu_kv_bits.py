@@ -105,3 +105,21 @@ def test_single_rows_hold_products_of_weight_and_value_scale(kv, dev, nh, n_kv, 
         c.v_scales[0, :, at] = 0.0
         got, want, mass, reach = single(kv, c, first, nh, p)
         assert ((got.double() - want).abs() <= R.tolerance(want, mass, reach, F32)).all(), at
+
+
+@pytest.mark.parametrize("t,nh,n_kv,hd,n_ctx,p", [(1, 1024, 256, 128, 512, 300), (1, 512, 256, 256, 512, 300),
+                                                  (9, 512, 256, 64, 512, 300), (9, 512, 256, 128, 512, 300),
+                                                  (1, 768, 256, 160, 512, 300)])
+def test_early_large_value_scales_cost_later_steps_nothing(kv, dev, t, nh, n_kv, hd, n_ctx, p):
+    """... in the general kernel: a warp's first step holds value scales 2^30 above the others', at negligible weights
+    (so many heads that cells are not split)."""
+    s = torch.zeros(p + t)
+    s[:128] = -60.0
+    c, first = scored(kv, dev, n_kv, hd, n_ctx, s)
+    c.v_scales[0] = 177 * 2.0 ** -24
+    c.v_scales[0, :, :128] = 32768.0
+    q = rows(dev, t, nh, hd, seed=78)
+    q[:, :, 0] = first
+    got = kv.attend(c, q, i32(dev, p), None, i32(dev, 0, t), t)
+    want, mass, reach = R.attend(c, q, [p], [0], [t], 0)
+    assert ((got.double() - want).abs() <= R.tolerance(want, mass, reach, F32)).all()
