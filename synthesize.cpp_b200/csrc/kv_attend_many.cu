@@ -10,7 +10,9 @@
 // parts for every type: with one, a tenth of the results of bf16 prompts were
 // rounded the other way, and a row's bits went by its call's length.  Key
 // scales of a tile and value scales of a group of tiles are first multiplied by
-// a power of two, so that fp16's range costs no bits.
+// a power of two that follows the largest, so that fp16's range costs no bits
+// to scales down to 2^-15 of the largest of their 64 cells; below, a value
+// scale is held to 2^-26 of it (a key's to 2^-32).
 //
 // Roles of the 16 warps, handing over through mbarriers: one warp fetches
 // 64-cell tiles of the cache by bulk copies and looks for what is seen of them
@@ -602,12 +604,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attend_many_kernel(const K
                 vtop = __reduce_max_sync(0xffffffffu, vtop);
                 all  = __all_sync(0xffffffffu, all);
                 odd  = __any_sync(0xffffffffu, odd);
-                // largest key operand below 2^15; values start 2^5 below that, and a new power is taken
-                // only when they would pass it
+                // largest key operand below 2^15; a tile's values lie up to 2^6 below that, and a new
+                // power (which begins a group: a fold) is taken only where they would not
                 const int kmax = ktop ? (int) (__float_as_uint(half_float((unsigned short) ktop)) >> 23) - 127 : 0;
                 const int vmax = vtop ? (int) (__float_as_uint(half_float((unsigned short) vtop)) >> 23) - 127 : -100;
-                if (vtop != 0u && (!v_set || vmax + v_exp > (V4 ? 11 : 7))) {
-                    v_exp = (V4 ? 6 : 2) - vmax;
+                constexpr int kHigh = V4 ? 11 : 7;  // scale below 2^(kHigh + 1), code up to 8 or 127
+                if (vtop != 0u && (!v_set || vmax + v_exp > kHigh || vmax + v_exp < kHigh - 6)) {
+                    v_exp = kHigh - 3 - vmax;
                     v_set = true;
                 }
                 __syncwarp();

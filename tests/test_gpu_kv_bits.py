@@ -123,3 +123,23 @@ def test_early_large_value_scales_cost_later_steps_nothing(kv, dev, t, nh, n_kv,
     got = kv.attend(c, q, i32(dev, p), None, i32(dev, 0, t), t)
     want, mass, reach = R.attend(c, q, [p], [0], [t], 0)
     assert ((got.double() - want).abs() <= R.tolerance(want, mass, reach, F32)).all()
+
+
+@pytest.mark.parametrize("bits_v", [4, 8])
+@pytest.mark.parametrize("nh,n_kv,hd", [(64, 32, 128), (64, 32, 64)])
+def test_prompts_after_early_large_value_scales(kv, dev, nh, n_kv, hd, bits_v):
+    """... and in the 128-row kernel, up and down more than once along the prefix."""
+    p, t = 500, 130
+    s = torch.zeros(p + t)
+    for first in (0, 192, 384):
+        s[first:first + 64] = -60.0
+    c, first = scored(kv, dev, n_kv, hd, 640, s, 8, bits_v)
+    c.v_scales[0] = 177 * 2.0 ** -24
+    c.v_scales[0, :, 0:64] = 32768.0
+    c.v_scales[0, :, 192:256] = 8.0
+    c.v_scales[0, :, 384:448] = 1000.0
+    q = rows(dev, t, nh, hd, seed=79)
+    q[:, :, 0] = first
+    got = kv.attend(c, q, i32(dev, p), None, i32(dev, 0, t), t)
+    want, mass, reach = R.attend(c, q, [p], [0], [t], 0)
+    assert ((got.double() - want).abs() <= R.tolerance(want, mass, reach, F32)).all()
