@@ -241,6 +241,15 @@ __global__ void __launch_bounds__(128)
                 }
             }
 
+            // an infinite scale: values of both signs, so the score is not a number
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+#pragma unroll
+                for (int h = 0; h < 2 * kHalf; ++h) {
+                    sc[n][h] = fmaf(sc[n][h], 0.0f, sc[n][h]);
+                }
+            }
+
             // ---- which of this thread's cells its rows see
             uint32_t seen[kHalf];  // bit 2n + j: cell 8n + 4j + c
 #pragma unroll

@@ -18,9 +18,10 @@
 // kMostWeight (the weights of cells whose values are zero must not overflow
 // either).  It is set so that the largest product of both is below 2^8, as far
 // as weights stay below 2^-kZero: 7 bits to grow, and a product's fp16 parts
-// hold it to 2^-22 of itself or 2^-32 of the largest.  So products add up in the tensor cores'
-// accumulators; they are moved to plain fp32 sums every kFold steps, because
-// the tensor cores cut their sums off where fp32 addition rounds.
+// hold it to 2^-22 of itself or 2^-32 of the largest.  So products add up in
+// the tensor cores' accumulators; they are moved to plain fp32 sums every kFold
+// steps, because the tensor cores cut their sums off where fp32 addition
+// rounds.
 //
 // 64 streams of 500 to 8100 positions (keys in 8 bits, values in 4; 519 MB):
 // 145 us, 3.6 TB/s; its copies alone take 85 us.  It is bound by instructions
@@ -230,7 +231,7 @@ __global__ void __maxnreg__(REGS) kv_attend_few_kernel(const KvAttendArgs a, con
                     for (int off = 4; off < 4 * NB; off <<= 1) {
                         v += __shfl_xor_sync(0xffffffffu, v, off);
                     }
-                    sc[x]    = v;
+                    sc[x]    = fmaf(v, 0.0f, v);  // an infinite scale: values of both signs, so not a number
                     vbits[x] = vd[(4 * x + c4) * nb];
                 }
             }

@@ -143,3 +143,16 @@ def test_prompts_after_early_large_value_scales(kv, dev, nh, n_kv, hd, bits_v):
     got = kv.attend(c, q, i32(dev, p), None, i32(dev, 0, t), t)
     want, mass, reach = R.attend(c, q, [p], [0], [t], 0)
     assert ((got.double() - want).abs() <= R.tolerance(want, mass, reach, F32)).all()
+
+
+@pytest.mark.parametrize("t,nh,n_kv,hd", [(1, 16, 8, 128), (1, 4, 2, 96), (1, 16, 2, 128), (9, 4, 2, 128), (3, 4, 2, 256),
+                                          (130, 64, 32, 128)])
+def test_an_infinite_key_scale_spoils_who_sees_it(kv, dev, t, nh, n_kv, hd):
+    """Codes of both signs times infinity: the score is not a number, whatever the codes' own sum."""
+    c = make(kv, dev, 1, 320, n_kv, hd, 8, 8, seed=80)
+    q = rows(dev, t, nh, hd, seed=81)
+    for p, hurt in ((100, t > 60), (160, True)):
+        c.k_scales[0, :, 160, 0] = float("inf")
+        got = kv.attend(c, q, i32(dev, p), None, i32(dev, 0, t), t)
+        bad = torch.arange(p, p + t, device=dev) >= 160
+        assert torch.isnan(got[bad]).all() and torch.isfinite(got[~bad]).all() and bool(bad.any()) == hurt
