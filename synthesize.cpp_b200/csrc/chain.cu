@@ -597,7 +597,8 @@ b200q8_status_t chain_create(const b200q8_chain_desc * desc, const b200q8_chain_
                              "chain_create_kv: types are Q4_0 or Q8_0, n_ctx a multiple of 64, window and sinks not "
                              "negative, n_head / n_kv at most 64");
         }
-        if (kv->ring && (kv->window == 0 || kv->sinks >= ad.n_ctx || kv->window + d.max_m - 1 > ad.n_ctx - kv->sinks)) {
+        if (kv->ring && (kv->window == 0 || kv->sinks >= ad.n_ctx || kv->window > ad.n_ctx ||
+                         kv->window + d.max_m - 1 > ad.n_ctx - kv->sinks)) {
             return set_error(B200Q8_ERR_INVALID_ARG, "chain_create_kv: a ring needs a window with window + max_m - 1 at "
                                                      "most n_ctx - sinks");
         }

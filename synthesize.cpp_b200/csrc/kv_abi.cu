@@ -197,7 +197,7 @@ b200q8_status_t b200q8_kv_attend(const b200q8_kv_cache * cache, const b200q8_kv_
     if (window < 0 || !std::isfinite(scale)) {
         return set_error(B200Q8_ERR_INVALID_ARG, "kv_attend: window must not be negative and scale finite");
     }
-    if (a.c.ring && (window == 0 || window + a.b.max_len - 1 > a.c.ring)) {
+    if (a.c.ring && (window == 0 || window > a.c.ring || window + a.b.max_len - 1 > a.c.ring)) {
         return set_error(B200Q8_ERR_INVALID_ARG,
                          "kv_attend: a ring cache needs a window, and window + max_len - 1 at most its %d cells",
                          a.c.ring);
