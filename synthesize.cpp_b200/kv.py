@@ -9,8 +9,9 @@ The cache's four arrays belong to the caller (``new_cache`` allocates them with 
 include/b200q8.h documents at b200q8_kv_cache.  Every call names its rows by runs of consecutive positions: run i is
 rows ``starts[i]:starts[i+1]`` at positions ``pos[i]``, ``pos[i] + 1``, ... of slot ``slots[i]``; without ``starts``
 each run is one row, without ``slots`` run i is slot i; ``max_len`` bounds the runs' lengths.  ``pos``, ``slots`` and
-``starts`` are int32 CUDA tensors.  Work is enqueued on torch's current stream; a failure raises B200Q8Error, and
-what only the device can see (a position outside the cache) is reported by ``q8.device_status``.
+``starts`` are int32 CUDA tensors.  Work is enqueued on torch's current stream of the cache's device, whichever device
+is current; a failure raises B200Q8Error, and what only the device can see (a position outside the cache) is reported by
+``q8.device_status``.
 """
 from __future__ import annotations
 
@@ -84,6 +85,15 @@ def _stream(cache: KVCache) -> int:
     return torch._C._cuda_getCurrentRawStream(cache._device)
 
 
+def _call(cache: KVCache, call, *args) -> None:
+    """The library launches on the current device: the cache's, for the time of the call."""
+    if torch._C._cuda_getDevice() == cache._device:
+        check(call(*args))
+    else:
+        with torch.cuda.device(cache._device):
+            check(call(*args))
+
+
 def _batch(cache: KVCache, n_tokens: int, pos, slots, starts, max_len: int) -> KVBatch:
     dev, i32 = cache._device, torch.int32
     n = pos.numel()
@@ -118,8 +128,8 @@ def write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, s
     if k.dtype != v.dtype or n != v.shape[0]:
         raise ValueError("kv.write: k and v must have one type and as many rows")
     ks, vs = _rows(cache, k, cache.n_kv, "k"), _rows(cache, v, cache.n_kv, "v")
-    check(lib().b200q8_kv_write(cache._desc, _batch(cache, n, pos, slots, starts, max_len), k.data_ptr(), ks,
-                                v.data_ptr(), vs, SRC_TYPES[k.dtype], _stream(cache)))
+    _call(cache, lib().b200q8_kv_write, cache._desc, _batch(cache, n, pos, slots, starts, max_len), k.data_ptr(), ks,
+          v.data_ptr(), vs, SRC_TYPES[k.dtype], _stream(cache))
 
 
 def read(cache: KVCache, n: int, pos: torch.Tensor, slots: torch.Tensor | None = None,
@@ -137,8 +147,8 @@ def read(cache: KVCache, n: int, pos: torch.Tensor, slots: torch.Tensor | None =
         ks, vs = _rows(cache, k, cache.n_kv, "out"), _rows(cache, v, cache.n_kv, "out")
     if k.dtype not in SRC_TYPES:
         raise ValueError("kv.read: dtype must be float32, float16 or bfloat16")
-    check(lib().b200q8_kv_read(cache._desc, _batch(cache, n, pos, slots, starts, max_len), k.data_ptr(), ks,
-                               v.data_ptr(), vs, SRC_TYPES[k.dtype], _stream(cache)))
+    _call(cache, lib().b200q8_kv_read, cache._desc, _batch(cache, n, pos, slots, starts, max_len), k.data_ptr(), ks,
+          v.data_ptr(), vs, SRC_TYPES[k.dtype], _stream(cache))
     return out
 
 
@@ -159,6 +169,6 @@ def attend(cache: KVCache, q: torch.Tensor, pos: torch.Tensor, slots: torch.Tens
         raise ValueError("kv.attend: out must have q's rows and type")
     else:
         os_ = _rows(cache, out, heads, "out")
-    check(lib().b200q8_kv_attend(cache._desc, _batch(cache, n, pos, slots, starts, max_len), q.data_ptr(), qs,
-                                 out.data_ptr(), os_, SRC_TYPES[q.dtype], heads, window, scale, _stream(cache)))
+    _call(cache, lib().b200q8_kv_attend, cache._desc, _batch(cache, n, pos, slots, starts, max_len), q.data_ptr(), qs,
+          out.data_ptr(), os_, SRC_TYPES[q.dtype], heads, window, scale, _stream(cache))
     return out

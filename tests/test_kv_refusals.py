@@ -34,3 +34,76 @@ def test_a_chain_refuses_every_window_that_passes_its_ring(abi, window):
     handle = ctypes.c_void_p()
     got = abi.lib().b200q8_chain_create_kv(ctypes.byref(desc), ctypes.byref(kvd), 0, ctypes.byref(handle))
     assert got == abi.ERR_INVALID_ARG and "ring" in abi.last_error()[1]
+
+
+# ------------------------------------------------------------------------------------------------ the Python module
+
+
+class OnDevice:
+    """A CPU tensor that says it is on device 1: enough for the module's checks."""
+
+    def __init__(self, t):
+        self.t = t
+
+    def get_device(self):
+        return 1
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+class Calls:
+    """The library's calls, recording the device that is current when they are made."""
+
+    def __init__(self, state):
+        self.state, self.seen = state, []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.seen.append((name, self.state["device"]))
+            return 0
+
+        return call
+
+
+@pytest.fixture()
+def two_devices(pkg, monkeypatch):
+    """(kv, a cache on device 1, the calls' record, the state whose "device" is current)."""
+    import torch
+    from synthesize_cpp_b200 import kv
+
+    state = {"device": 0}
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, state["device"] = state["device"], self.index
+
+        def __exit__(self, *_):
+            state["device"] = self.before
+
+    lib = Calls(state)
+    monkeypatch.setattr(kv, "lib", lambda: lib)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["device"])
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: state["device"])
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index)
+    c = object.__new__(kv.KVCache)
+    c.n_kv, c.head_dim, c._device, c._desc = 2, 64, 1, None
+    return kv, c, lib, state
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_calls_run_on_the_caches_device(two_devices, current):
+    import torch
+
+    kv, c, lib, state = two_devices
+    state["device"] = current
+    x, p = OnDevice(torch.zeros((1, 2, 64))), OnDevice(torch.zeros(1, dtype=torch.int32))
+    kv.write(c, x, x, p)
+    kv.read(c, 1, p, out=(x, x))
+    kv.attend(c, x, p, out=x)
+    assert lib.seen == [("b200q8_kv_write", 1), ("b200q8_kv_read", 1), ("b200q8_kv_attend", 1)]
+    assert state["device"] == current
