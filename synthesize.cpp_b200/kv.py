@@ -8,10 +8,10 @@
 The cache's four arrays belong to the caller (``new_cache`` allocates them with torch); their layout is the one
 include/b200q8.h documents at b200q8_kv_cache.  Every call names its rows by runs of consecutive positions: run i is
 rows ``starts[i]:starts[i+1]`` at positions ``pos[i]``, ``pos[i] + 1``, ... of slot ``slots[i]``; without ``starts``
-each run is one row, without ``slots`` run i is slot i; ``max_len`` bounds the runs' lengths.  ``pos``, ``slots`` and
-``starts`` are int32 CUDA tensors.  Work is enqueued on torch's current stream of the cache's device, whichever device
-is current; a failure raises B200Q8Error, and what only the device can see (a position outside the cache) is reported by
-``q8.device_status``.
+each run is one row, without ``slots`` run i is slot i; ``max_len`` bounds the runs' lengths (left out, the number of rows does; a close bound
+makes a faster call).  ``pos``, ``slots`` and ``starts`` are int32 CUDA tensors.  Work is enqueued on torch's current
+stream of the cache's device, whichever device is current; a failure raises B200Q8Error, and what only the device can see
+(a position outside the cache) is reported by ``q8.device_status``.
 """
 from __future__ import annotations
 
@@ -94,7 +94,7 @@ def _call(cache: KVCache, call, *args) -> None:
             check(call(*args))
 
 
-def _batch(cache: KVCache, n_tokens: int, pos, slots, starts, max_len: int) -> KVBatch:
+def _batch(cache: KVCache, n_tokens: int, pos, slots, starts, max_len: int | None, window: int = 1) -> KVBatch:
     dev, i32 = cache._device, torch.int32
     n = pos.numel()
     # dense vectors of int32 on the cache's device
@@ -104,6 +104,11 @@ def _batch(cache: KVCache, n_tokens: int, pos, slots, starts, max_len: int) -> K
             or starts is not None and (starts.dtype != i32 or starts.get_device() != dev or starts.dim() != 1
                                        or starts.numel() != n + 1 or not starts.is_contiguous())):
         raise ValueError("kv: pos, slots [n] and starts [n + 1] must be dense int32 tensors on the cache's device")
+    if max_len is None:  # no run is longer than all rows, and in a ring than its cells allow
+        max_len = 1 if starts is None else n_tokens
+        if cache.ring:
+            max_len = min(max_len, cache.n_ctx - cache.sinks - window + 1)
+        max_len = max(1, max_len)
     return KVBatch(n, n_tokens, max_len, None if starts is None else starts.data_ptr(), pos.data_ptr(),
                    None if slots is None else slots.data_ptr())
 
@@ -122,7 +127,7 @@ def _rows(cache: KVCache, t: torch.Tensor, heads: int, what: str) -> int:
 
 
 def write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor | None = None,
-          starts: torch.Tensor | None = None, max_len: int = 1) -> None:
+          starts: torch.Tensor | None = None, max_len: int | None = None) -> None:
     """Quantises rows k, v [n, n_kv, head_dim] (row-strided views allowed) into their cells."""
     n = k.shape[0]
     if k.dtype != v.dtype or n != v.shape[0]:
@@ -133,7 +138,7 @@ def write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, s
 
 
 def read(cache: KVCache, n: int, pos: torch.Tensor, slots: torch.Tensor | None = None,
-         starts: torch.Tensor | None = None, max_len: int = 1, dtype: torch.dtype = torch.float32,
+         starts: torch.Tensor | None = None, max_len: int | None = None, dtype: torch.dtype = torch.float32,
          out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The n rows of the runs as values: (k, v), each [n, n_kv, head_dim]."""
     if out is None:
@@ -153,7 +158,7 @@ def read(cache: KVCache, n: int, pos: torch.Tensor, slots: torch.Tensor | None =
 
 
 def attend(cache: KVCache, q: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor | None = None,
-           starts: torch.Tensor | None = None, max_len: int = 1, window: int = 0, scale: float = 0.0,
+           starts: torch.Tensor | None = None, max_len: int | None = None, window: int = 0, scale: float = 0.0,
            out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q [n, n_head, head_dim] over the cached positions each row sees; returns [n, n_head, head_dim] in
     q's type.  window 0 sees the whole prefix; scale 0 means 1/sqrt(head_dim)."""
@@ -169,6 +174,6 @@ def attend(cache: KVCache, q: torch.Tensor, pos: torch.Tensor, slots: torch.Tens
         raise ValueError("kv.attend: out must have q's rows and type")
     else:
         os_ = _rows(cache, out, heads, "out")
-    _call(cache, lib().b200q8_kv_attend, cache._desc, _batch(cache, n, pos, slots, starts, max_len), q.data_ptr(), qs,
+    _call(cache, lib().b200q8_kv_attend, cache._desc, _batch(cache, n, pos, slots, starts, max_len, window), q.data_ptr(), qs,
           out.data_ptr(), os_, SRC_TYPES[q.dtype], heads, window, scale, _stream(cache))
     return out

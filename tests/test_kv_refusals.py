@@ -56,11 +56,12 @@ class Calls:
     """The library's calls, recording the device that is current when they are made."""
 
     def __init__(self, state):
-        self.state, self.seen = state, []
+        self.state, self.seen, self.batches = state, [], []
 
     def __getattr__(self, name):
         def call(*args):
             self.seen.append((name, self.state["device"]))
+            self.batches.append(args[1])
             return 0
 
         return call
@@ -70,7 +71,7 @@ class Calls:
 def two_devices(pkg, monkeypatch):
     """(kv, a cache on device 1, the calls' record, the state whose "device" is current)."""
     import torch
-    from synthesize_cpp_b200 import kv
+    from synthesize_cpp_b200 import _abi, kv
 
     state = {"device": 0}
 
@@ -91,7 +92,8 @@ def two_devices(pkg, monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: state["device"])
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index)
     c = object.__new__(kv.KVCache)
-    c.n_kv, c.head_dim, c._device, c._desc = 2, 64, 1, None
+    c.n_kv, c.head_dim, c._device = 2, 64, 1
+    c._desc = _abi.KVCacheDesc(8, 8, 16, 128, 2, 64, 4, 0, 4096, 4096, 4096, 4096)
     return kv, c, lib, state
 
 
@@ -107,3 +109,28 @@ def test_calls_run_on_the_caches_device(two_devices, current):
     kv.attend(c, x, p, out=x)
     assert lib.seen == [("b200q8_kv_write", 1), ("b200q8_kv_read", 1), ("b200q8_kv_attend", 1)]
     assert state["device"] == current
+
+
+def test_runs_without_max_len_are_bounded_by_the_rows(two_devices):
+    """A caller who names runs and no bound gets every row, not zeros beyond the first of each run."""
+    import torch
+
+    kv, c, lib, _ = two_devices
+    ints = lambda *v: OnDevice(torch.tensor(v, dtype=torch.int32))  # noqa: E731
+    x, p, starts = OnDevice(torch.zeros((5, 2, 64))), ints(0, 9), ints(0, 3, 5)
+    kv.write(c, x, x, p, None, starts)
+    kv.read(c, 5, p, None, starts, out=(x, x))
+    kv.attend(c, x, p, starts=starts, out=x)
+    assert [b.max_len for b in lib.batches] == [5, 5, 5]
+    kv.attend(c, x, p, None, starts, 3, out=x)
+    kv.attend(c, OnDevice(torch.zeros((2, 2, 64))), p, out=OnDevice(torch.zeros((2, 2, 64))))
+    assert [b.max_len for b in lib.batches[3:]] == [3, 1]
+    none = OnDevice(torch.zeros((0, 2, 64)))
+    kv.attend(c, none, p, None, ints(0, 0, 0), out=none)
+    assert lib.batches[-1].max_len == 1
+    c._desc.ring = 1  # 124 cells go round
+    x = OnDevice(torch.zeros((200, 2, 64)))
+    kv.write(c, x, x, p, None, starts)
+    kv.attend(c, x, p, None, starts, window=100, out=x)
+    kv.attend(c, x, p, None, starts, window=124, out=x)
+    assert [b.max_len for b in lib.batches[-3:]] == [124, 25, 1]
