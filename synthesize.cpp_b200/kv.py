@@ -69,6 +69,8 @@ class KVCache:
 def new_cache(n_slots: int, n_ctx: int, n_kv: int, head_dim: int, type_k: int = KV_Q8_0, type_v: int = KV_Q8_0,
               sinks: int = 0, ring: bool = False, device: torch.device | str = "cuda") -> KVCache:
     """Allocates a cache (n_ctx is rounded up to a multiple of 64)."""
+    if head_dim % 32 != 0 or not 32 <= head_dim <= 256:
+        raise ValueError("new_cache: head_dim must be a multiple of 32 up to 256")
     n_ctx = (n_ctx + 63) // 64 * 64
     arrays = []
     for t in (type_k, type_v):

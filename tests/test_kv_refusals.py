@@ -134,3 +134,13 @@ def test_runs_without_max_len_are_bounded_by_the_rows(two_devices):
     kv.attend(c, x, p, None, starts, window=100, out=x)
     kv.attend(c, x, p, None, starts, window=124, out=x)
     assert [b.max_len for b in lib.batches[-3:]] == [124, 25, 1]
+
+
+@pytest.mark.parametrize("head_dim", [33, 63, 0, 16, 48, 288, -32])
+def test_new_cache_refuses_other_head_sizes(pkg, head_dim):
+    """... 33 in four bits is 16 bytes a row, as 32 is."""
+    from synthesize_cpp_b200 import kv
+
+    for t in (kv.KV_Q4_0, kv.KV_Q8_0):
+        with pytest.raises(ValueError, match="multiple of 32"):
+            kv.new_cache(1, 64, 1, head_dim, t, t, device="cpu")
