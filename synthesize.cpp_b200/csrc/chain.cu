@@ -766,9 +766,9 @@ b200q8_status_t chain_create(const b200q8_chain_desc * desc, const b200q8_chain_
             c->owned.push_back(p3);
             c->k_rot = static_cast<float *>(p3);
         }
-        if (e == cudaSuccess) {  // the kernel's attributes, before any capture
+        for (int64_t m = 1; m <= d.max_m && e == cudaSuccess; ++m) {  // the kernels' attributes, before any capture
             AttnArgs aa = {};
-            e           = prepare_kv_attend(c->kv_attend_args(0, aa, 0, 1));
+            e           = prepare_kv_attend(c->kv_attend_args(0, aa, 0, m), c->sms);
         }
     }
     // persistent step (M <= 2): per-layer weight table, LL hand-off words,

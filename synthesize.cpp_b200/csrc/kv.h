@@ -64,7 +64,7 @@ struct KvAttendMany {
 };
 KvAttendMany kv_attend_many(int nb, int k4, int v4, int type);
 // Sets the attributes of the kernel that such a call launches (launches do it too; a capture should not).
-cudaError_t  prepare_kv_attend(const KvAttendArgs & a);
+cudaError_t  prepare_kv_attend(const KvAttendArgs & a, int sm_count);
 cudaError_t  launch_kv_attend(const KvAttendArgs & a, cudaStream_t stream, int sm_count);
 
 // The cache kernels' status word on the current device (their translation unit has one of its own; the first error

@@ -616,8 +616,8 @@ AttendPlan attend_plan(const KvAttendArgs & a, int sm_count) {
 
 }  // namespace
 
-cudaError_t prepare_kv_attend(const KvAttendArgs & a) {
-    return prepare_kernel(attend_plan(a, 148).fn);
+cudaError_t prepare_kv_attend(const KvAttendArgs & a, int sm_count) {
+    return prepare_kernel(attend_plan(a, sm_count).fn);
 }
 
 cudaError_t launch_kv_attend(const KvAttendArgs & args, cudaStream_t stream, int sm_count) {

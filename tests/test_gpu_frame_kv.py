@@ -1,6 +1,8 @@
-"""Steps with output heads and frames over quantised caches: what b200q8_chain_create_kv's chains share
+"""Steps with output heads, frames and long caches over quantised caches: what b200q8_chain_create_kv's chains share
 with the others."""
 from __future__ import annotations
+
+import importlib
 
 import numpy as np
 import pytest
@@ -8,10 +10,15 @@ import torch
 
 from test_gpu_attention import THETA, qk_norms
 from test_gpu_chain import EPS, H, HD, I, NH, NKV, make_model, upload
-from test_gpu_chain_kv import i32
+from test_gpu_chain_kv import build, check_layer, i32
 from test_gpu_frame import G, PV, TV, rms_norm, t
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def kv(pkg):
+    return importlib.import_module("synthesize_cpp_b200.kv")
 
 
 def stack(O, chain_mod, dev, seed, vocab, n_heads, table_rows, n_slots, max_m, kvd):
@@ -98,3 +105,23 @@ def test_frames(chain_mod, frame_mod, O, q8, dev, m):
     fr.close()
     for ch in (talker, pred, talker2, pred2):
         ch.close()
+
+
+def test_long_caches_at_every_batch_size(pkg, O, kv, chain_mod, q8, dev):
+    """4096 cells a slot: steps of one token and of more take kernels of their own, each first met in a capture (the
+    positions stay where check_layer's bound on the rotation holds)."""
+    ch, qkn = build(O, chain_mod, dev, 1, 12, 4096, 6, 2600, dict(type_k=8, type_v=8))
+    c = ch.kv_cache(0)
+    k = torch.randn((60, NKV, HD), device=dev)
+    for s in range(6):
+        kv.write(c, k.roll(s, 0), k.roll(-s, 0), i32(dev, [0]), i32(dev, [s]), i32(dev, [0, 60]), 60)
+    rng = np.random.default_rng(9)
+    for step, m in enumerate((2, 1, 5, 3, 4, 6)):
+        pos, slots = [60 - 7 * i + step for i in range(m)], [(5 * i + step) % 6 for i in range(m)]
+        x = torch.from_numpy(rng.standard_normal((m, H)).astype(np.float32)).to(dev)
+        h = torch.empty((m, H), device=dev)
+        ch.run_at(i32(dev, rng.integers(0, 64, m)), x, i32(dev, pos), h, slots=i32(dev, slots))
+        torch.cuda.synchronize(dev)
+        check_layer(O, kv, ch, qkn, 0, m, pos, slots, 0, dev)
+    assert q8.device_status(0, clear=True) == 0
+    ch.close()
