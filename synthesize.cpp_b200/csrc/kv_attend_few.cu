@@ -7,11 +7,13 @@
 // head gives every block's sum in a row - a lane - of its own.  A lane scales
 // its one block's sums, the blocks are added by shuffles, and each lane then
 // forms the weights times its own block's value scales, once, instead of
-// every lane doing so for every block.  q is scaled by a power of two to 22
-// bits and sign and enters as three signed bytes: the keys' codes are bytes as
-// they lie (nibbles: a mask), the sums are exact integers.  The second product,
-// in fp16, gives row (h, b) the values of all blocks; those of block b count.
-// Rows 8 .. 15 hold the weights' second fp16 parts (of q: the second byte).
+// every lane doing so for every block.  q is scaled by a power of two to 30
+// bits and sign and enters as four signed bytes: the keys' codes are bytes as
+// they lie (nibbles: a mask), the sums are exact integers.  (Fixed point: three
+// bytes would hold a value 2^10 below the row's largest to 12 bits.)  The
+// second product, in fp16, gives row (h, b) the values of all blocks; those of
+// block b count.  Rows 8 .. 15 hold the weights' second fp16 parts (of q: the
+// third and first bytes).
 //
 // The reference of the weights moves only when the largest weight times the
 // largest value scale of a lane's cells would pass 2^15, or a weight
@@ -84,14 +86,14 @@ __global__ void __maxnreg__(REGS) kv_attend_few_kernel(const KvAttendArgs a, con
     }
 
     // ---- this lane's operand row: query row t.row + g / NB, block g % NB, as
-    // q * 2^x in three signed bytes (22 bits and sign)
+    // q * 2^x in four signed bytes (30 bits and sign)
     const int  block = g % NB;
     const int  row   = t.row + g / NB;
     const bool valid = row < t.n_rows && block < nb;
     const int  token = row < t.n_rows ? row / a.group : 0;
     const int  es    = a.type == kSrcF32 ? 4 : 2;
     const int  prow = row < t.n_rows ? t.r.pos + token : -1, lrow = a.window ? prow - a.window : -1;
-    uint32_t   qhi[NB][4], qlo[NB][4];  // rows g: parts 2 | 0, rows g + 8: part 1 | none
+    uint32_t   qhi[NB][4], qlo[NB][4];  // rows g: parts 3 | 1, rows g + 8: parts 2 | 0
     int        chi[4], clo[4];          // what the sums start from
     float      unscale;
     {
@@ -116,45 +118,45 @@ __global__ void __maxnreg__(REGS) kv_attend_few_kernel(const KvAttendArgs a, con
             bad = __shfl_xor_sync(0xffffffffu, (int) bad, off) != 0 || bad;
         }
         float up;
-        row_scale(top, a.scale, 22, up, unscale);
+        row_scale(top, a.scale, 30, up, unscale);
         if (bad) {
             unscale = NAN;  // every score of the row
         }
-        uint32_t part[3][2] = {};
-        int      total[3]   = {};
+        uint32_t part[4][2] = {};
+        int      total[4]   = {};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             // the lane's codes: even and odd nibbles of a word, or two words of bytes
             const int reg = K4 ? e & 1 : e >> 2, byte = K4 ? e >> 1 : e & 3;
             int       v   = bad ? 0 : __float2int_rn(q[e] * up);
 #pragma unroll
-            for (int k = 0; k < 3; ++k) {
-                const int digit = k == 2 ? v : (int) (signed char) (v & 0xff);
+            for (int k = 0; k < 4; ++k) {
+                const int digit = k == 3 ? v : (int) (signed char) (v & 0xff);
                 part[k][reg] |= (uint32_t) (digit & 0xff) << (8 * byte);
                 total[k] += digit;
                 v = (v - digit) >> 8;
             }
         }
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
+        for (int k = 0; k < 4; ++k) {
             total[k] += __shfl_xor_sync(0xffffffffu, total[k], 1);
             total[k] += __shfl_xor_sync(0xffffffffu, total[k], 2);
         }
         const int off = K4 ? 8 : 0;  // Q4_0 codes are stored as code + 8
-        chi[0] = chi[1] = kBias - off * total[2];
-        chi[2] = chi[3] = kBias - off * total[1];
-        clo[0] = clo[1] = kBias - off * total[0];
-        clo[2] = clo[3] = 0;
+        chi[0] = chi[1] = kBias - off * total[3];
+        chi[2] = chi[3] = kBias - off * total[2];
+        clo[0] = clo[1] = kBias - off * total[1];
+        clo[2] = clo[3] = kBias - off * total[0];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            qhi[b][0] = b == block ? part[2][0] : 0u;
-            qhi[b][1] = b == block ? part[1][0] : 0u;
-            qhi[b][2] = b == block ? part[2][1] : 0u;
-            qhi[b][3] = b == block ? part[1][1] : 0u;
-            qlo[b][0] = b == block ? part[0][0] : 0u;
-            qlo[b][1] = 0u;
-            qlo[b][2] = b == block ? part[0][1] : 0u;
-            qlo[b][3] = 0u;
+            qhi[b][0] = b == block ? part[3][0] : 0u;
+            qhi[b][1] = b == block ? part[2][0] : 0u;
+            qhi[b][2] = b == block ? part[3][1] : 0u;
+            qhi[b][3] = b == block ? part[2][1] : 0u;
+            qlo[b][0] = b == block ? part[1][0] : 0u;
+            qlo[b][1] = b == block ? part[0][0] : 0u;
+            qlo[b][2] = b == block ? part[1][1] : 0u;
+            qlo[b][3] = b == block ? part[0][1] : 0u;
         }
     }
     const int pos_lo = t.r.pos + t.row / a.group, pos_hi = t.r.pos + t.last / a.group;
@@ -223,9 +225,9 @@ __global__ void __maxnreg__(REGS) kv_attend_few_kernel(const KvAttendArgs a, con
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                     const int   u = y >> 1, j = y & 1, x = 2 * u0 + y;
-                    const float s2 = __int_as_float(hi[u][j]) - 12582912.0f, s1 = __int_as_float(hi[u][j + 2]) - 12582912.0f;
-                    const float s0 = __int_as_float(lo[u][j]) - 12582912.0f;
-                    float       v  = fmaf(s2, 65536.0f, fmaf(s1, 256.0f, s0)) * half_float(kd[(4 * x + c4) * nb]);
+                    const float s3 = __int_as_float(hi[u][j]) - 12582912.0f, s2 = __int_as_float(hi[u][j + 2]) - 12582912.0f;
+                    const float s1 = __int_as_float(lo[u][j]) - 12582912.0f, s0 = __int_as_float(lo[u][j + 2]) - 12582912.0f;
+                    float       v  = fmaf(fmaf(s3, 256.0f, s2), 65536.0f, fmaf(s1, 256.0f, s0)) * half_float(kd[(4 * x + c4) * nb]);
                     v              = EXACT || block < nb ? v : 0.0f;
 #pragma unroll
                     for (int off = 4; off < 4 * NB; off <<= 1) {

@@ -156,3 +156,23 @@ def test_an_infinite_key_scale_spoils_who_sees_it(kv, dev, t, nh, n_kv, hd):
         got = kv.attend(c, q, i32(dev, p), None, i32(dev, 0, t), t)
         bad = torch.arange(p, p + t, device=dev) >= 160
         assert torch.isnan(got[bad]).all() and torch.isfinite(got[~bad]).all() and bool(bad.any()) == hurt
+
+
+@pytest.mark.parametrize("bits_k", [4, 8])
+@pytest.mark.parametrize("nh,n_kv,hd,n_ctx,p", SINGLES)
+def test_a_strong_query_channel_that_keys_do_not_meet(kv, dev, nh, n_kv, hd, n_ctx, p, bits_k):
+    """A value of q 2^12 times the others where keys are zero: the others keep their bits."""
+    c = make(kv, dev, 1, n_ctx, n_kv, hd, bits_k, 8, seed=90)
+    at = R.places(hd, 4)[7]
+    if bits_k == 8:
+        c.k_codes[..., at] = 0
+    else:
+        byte = c.k_codes[..., at // 2]
+        c.k_codes[..., at // 2] = byte & (0x0f if at % 2 else 0xf0) | (0x80 if at % 2 else 0x08)
+    c.k_scales[:] *= 4.0
+    q = rows(dev, 1, nh, hd, seed=91)
+    q[:, :, 7] = 4096.0
+    got = kv.attend(c, q, i32(dev, p))
+    want, mass, reach = R.attend(c, q, [p], [0], [1], 0)
+    err, tol = (got.double() - want).abs(), R.tolerance(want, mass, reach, F32)
+    assert (err <= tol).all(), float((err / tol).max())
