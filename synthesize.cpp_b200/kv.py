@@ -82,20 +82,6 @@ def new_cache(n_slots: int, n_ctx: int, n_kv: int, head_dim: int, type_k: int = 
     return KVCache(*arrays, sinks=sinks, ring=ring)
 
 
-def _stream(cache: KVCache) -> int:
-    """torch's current stream of the cache's device (the raw handle: a step's calls are short)."""
-    return torch._C._cuda_getCurrentRawStream(cache._device)
-
-
-def _call(cache: KVCache, call, *args) -> None:
-    """The library launches on the current device: the cache's, for the time of the call."""
-    if torch._C._cuda_getDevice() == cache._device:
-        check(call(*args))
-    else:
-        with torch.cuda.device(cache._device):
-            check(call(*args))
-
-
 def _batch(cache: KVCache, n_tokens: int, pos, slots, starts, max_len: int | None, window: int = 1) -> KVBatch:
     dev, i32 = cache._device, torch.int32
     n = pos.numel()
@@ -106,12 +92,12 @@ def _batch(cache: KVCache, n_tokens: int, pos, slots, starts, max_len: int | Non
             or starts is not None and (starts.dtype != i32 or starts.get_device() != dev or starts.dim() != 1
                                        or starts.numel() != n + 1 or not starts.is_contiguous())):
         raise ValueError("kv: pos, slots [n] and starts [n + 1] must be dense int32 tensors on the cache's device")
+    if starts is None:
+        return KVBatch(n, n_tokens, 1, None, pos.data_ptr(), None if slots is None else slots.data_ptr())
     if max_len is None:  # no run is longer than all rows, and in a ring than its cells allow
-        max_len = 1 if starts is None else n_tokens
-        if cache.ring:
-            max_len = min(max_len, cache.n_ctx - cache.sinks - window + 1)
-        max_len = max(1, max_len)
-    return KVBatch(n, n_tokens, max_len, None if starts is None else starts.data_ptr(), pos.data_ptr(),
+        most = cache.n_ctx - cache.sinks - window + 1 if cache.ring else n_tokens
+        max_len = max(1, min(n_tokens, most))
+    return KVBatch(n, n_tokens, max_len, starts.data_ptr(), pos.data_ptr(),
                    None if slots is None else slots.data_ptr())
 
 
@@ -131,18 +117,26 @@ def _rows(cache: KVCache, t: torch.Tensor, heads: int, what: str) -> int:
 def write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor | None = None,
           starts: torch.Tensor | None = None, max_len: int | None = None) -> None:
     """Quantises rows k, v [n, n_kv, head_dim] (row-strided views allowed) into their cells."""
+    dev = cache._device
+    if torch._C._cuda_getDevice() != dev:  # the library launches on the current device
+        with torch.cuda.device(dev):
+            return write(cache, k, v, pos, slots, starts, max_len)
     n = k.shape[0]
     if k.dtype != v.dtype or n != v.shape[0]:
         raise ValueError("kv.write: k and v must have one type and as many rows")
     ks, vs = _rows(cache, k, cache.n_kv, "k"), _rows(cache, v, cache.n_kv, "v")
-    _call(cache, lib().b200q8_kv_write, cache._desc, _batch(cache, n, pos, slots, starts, max_len), k.data_ptr(), ks,
-          v.data_ptr(), vs, SRC_TYPES[k.dtype], _stream(cache))
+    check(lib().b200q8_kv_write(cache._desc, _batch(cache, n, pos, slots, starts, max_len), k.data_ptr(), ks,
+                                v.data_ptr(), vs, SRC_TYPES[k.dtype], torch._C._cuda_getCurrentRawStream(dev)))
 
 
 def read(cache: KVCache, n: int, pos: torch.Tensor, slots: torch.Tensor | None = None,
          starts: torch.Tensor | None = None, max_len: int | None = None, dtype: torch.dtype = torch.float32,
          out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The n rows of the runs as values: (k, v), each [n, n_kv, head_dim]."""
+    dev = cache._device
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return read(cache, n, pos, slots, starts, max_len, dtype, out)
     if out is None:
         both = cache.k_scales.new_empty((2, n, cache.n_kv, cache.head_dim), dtype=dtype)
         k, v = out = both.unbind(0)
@@ -154,8 +148,8 @@ def read(cache: KVCache, n: int, pos: torch.Tensor, slots: torch.Tensor | None =
         ks, vs = _rows(cache, k, cache.n_kv, "out"), _rows(cache, v, cache.n_kv, "out")
     if k.dtype not in SRC_TYPES:
         raise ValueError("kv.read: dtype must be float32, float16 or bfloat16")
-    _call(cache, lib().b200q8_kv_read, cache._desc, _batch(cache, n, pos, slots, starts, max_len), k.data_ptr(), ks,
-          v.data_ptr(), vs, SRC_TYPES[k.dtype], _stream(cache))
+    check(lib().b200q8_kv_read(cache._desc, _batch(cache, n, pos, slots, starts, max_len), k.data_ptr(), ks,
+                               v.data_ptr(), vs, SRC_TYPES[k.dtype], torch._C._cuda_getCurrentRawStream(dev)))
     return out
 
 
@@ -164,6 +158,10 @@ def attend(cache: KVCache, q: torch.Tensor, pos: torch.Tensor, slots: torch.Tens
            out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q [n, n_head, head_dim] over the cached positions each row sees; returns [n, n_head, head_dim] in
     q's type.  window 0 sees the whole prefix; scale 0 means 1/sqrt(head_dim)."""
+    dev = cache._device
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return attend(cache, q, pos, slots, starts, max_len, window, scale, out)
     shape = q.shape
     if len(shape) != 3:
         raise ValueError("kv.attend: q must be [n, n_head, head_dim]")
@@ -176,6 +174,6 @@ def attend(cache: KVCache, q: torch.Tensor, pos: torch.Tensor, slots: torch.Tens
         raise ValueError("kv.attend: out must have q's rows and type")
     else:
         os_ = _rows(cache, out, heads, "out")
-    _call(cache, lib().b200q8_kv_attend, cache._desc, _batch(cache, n, pos, slots, starts, max_len, window), q.data_ptr(), qs,
-          out.data_ptr(), os_, SRC_TYPES[q.dtype], heads, window, scale, _stream(cache))
+    check(lib().b200q8_kv_attend(cache._desc, _batch(cache, n, pos, slots, starts, max_len, window), q.data_ptr(), qs,
+                                 out.data_ptr(), os_, SRC_TYPES[q.dtype], heads, window, scale, torch._C._cuda_getCurrentRawStream(dev)))
     return out
