@@ -422,14 +422,17 @@ void b200q8_frame_destroy(b200q8_frame * frame);
 /* Block types of cached rows (ggml type ids).  Both hold a row as blocks of
  * 32 values with one fp16 scale each; a value is read back as code * scale.
  *   Q8_0  d = max|x| * (1/127), code = x * (1/d) rounded half away from zero
- *         (b200q8_quantize_rows divides by 127: its d may differ in the last
- *         fp32 bit, so that a code next to a tie may be one off; NaN and
+ *         (b200q8_quantize_rows, as ggml, divides by 127: in 4 blocks of 100
+ *         d differs in the last fp32 bit, so that a code next to a tie may be
+ *         one off theirs; neither is nearer to exact arithmetic.  NaN and
  *         infinities are treated as there)
  *   Q4_0  d = m / -8 with m the first value of largest magnitude,
  *         code = min(15, floor(x * (1/d) + 8.5)) - 8, in -8..7
  * computed in fp32 against the scale before it is rounded to fp16.  A Q4_0
  * block that holds a NaN or an infinity gets a NaN scale and reads back as
- * NaN; a scale beyond fp16's range is stored as infinity. */
+ * NaN; a scale beyond fp16's range is stored as infinity (values read back as
+ * infinities and NaN; a row that sees such a key is NaN, and the block of such
+ * a value). */
 #define B200Q8_KV_Q4_0 2
 #define B200Q8_KV_Q8_0 8
 
@@ -468,7 +471,7 @@ typedef struct b200q8_kv_cache {
  * least the longest run; runs may be empty.  A run with a bad entry (slot or
  * position outside the cache, length negative or above max_len, rows outside
  * n_tokens) records B200Q8_ERR_INVALID_ARG in the device status; write skips
- * it, read and attend zero its rows. */
+ * it, read and attend zero its rows.  Rows that no run names are left alone. */
 typedef struct b200q8_kv_batch {
     int64_t         n_seqs;   /* up to 65535 */
     int64_t         n_tokens;
@@ -503,12 +506,16 @@ b200q8_status_t b200q8_kv_read(const b200q8_kv_cache * cache, const b200q8_kv_ba
  * window > 0, j > p - window or j < cache->sinks.  The rows j of the run
  * itself must be in the cache (b200q8_kv_write before it on the stream).
  * q and out rows are n_head * head_dim values, type B200Q8_SRC_* for both;
- * scale 0 means 1/sqrt(head_dim).  Scores, softmax and sums are fp32; q and
- * the weights enter the tensor cores with 22 bits (as integer or fp16 parts)
- * and codes and scales exactly, so F32 results are as exact as plain fp32 ones,
- * and 16-bit ones such results rounded once.  A weight is held to 2^-22 of itself or
- * 2^-32 of the row's largest, whichever is more.  Cells a row does not see
- * never contribute, whatever they hold.  On a ring cache a window is required and
+ * scale 0 means 1/sqrt(head_dim).  Scores, softmax and sums are fp32 and codes
+ * enter the tensor cores exactly.  q is held to 2^-22 of each value or 2^-30 of
+ * the row's largest, whichever is more; a weight times its cell's value scale to
+ * 2^-21 of itself, or 2^-32 of the largest such weight times the largest such
+ * scale (in runs of 128 query rows a kv head and more: weights to 2^-32 of the
+ * largest, and value scales exactly down to 2^-15 of the largest of 64
+ * neighbouring cells, to 2^-26 of it below).  So F32 results are as exact as
+ * plain fp32 ones and 16-bit ones are such results rounded once, except where
+ * scales differ by more than that.  Cells a row does not see never contribute,
+ * whatever they hold.  On a ring cache a window is required and
  * window + max_len - 1 may not pass n_ctx - sinks.  n_head / n_kv <= 64.
  * No scratch memory, one launch, deterministic.  Replaces the mul_mat /
  * soft_max / mul_mat of src/arch/qwen3-tts/operations.cpp:86-135 over such a

@@ -36,8 +36,8 @@
 // that the columns a thread has scores of are the cells whose values it loads:
 // column 2c + i of 8-column tile u of 16-cell group s is cell 16s+8u+4i+c.
 //
-// 24 streams, 24 heads over 4 of 64 values, 8-bit, bf16 (38 MB): 24 us a call,
-// 1.6 TB/s; one wave of clusters, bound by the chain of a step (codes to fp16,
+// 24 streams, 24 heads over 4 of 64 values, 8-bit, bf16 (38 MB): 25 us a call,
+// 1.5 TB/s; one wave of clusters, bound by the chain of a step (codes to fp16,
 // two products with a reduction between them) rather than by the copies.
 #include "kv_attend.cuh"
 
@@ -590,14 +590,20 @@ AttendPlan attend_plan(const KvAttendArgs & a, int sm_count) {
     p.tiles = (rows + high * p.wr - 1) / (high * p.wr);
     const int64_t base  = p.tiles * a.c.n_kv * a.b.n_seqs;
     const int64_t reach = a.window ? std::min((int64_t) a.c.n_ctx, (int64_t) a.window + a.b.max_len + a.c.sinks) : a.c.n_ctx;
-    // Three CTAs of four warps fit an SM.  While the rows leave slots free the
-    // cells are split over a cluster, so that one wave takes the call: 8 kv
+    // Slots are counted as three CTAs of four warps an SM, which is what fits at
+    // 168 registers a thread or fewer (the few-row kernel, heads of 64).  Of the
+    // forms with up to 255 two fit (heads of 128 in 16-row tiles, heads of more
+    // blocks), of heads of 256 in 8 bits one (139 KB of stages); there a call
+    // near the count takes a second wave.
+    // While the rows leave slots free the cells are split over a cluster: 8 kv
     // heads of one stream over 32701 cells take 420 us unsplit and 41 us over
     // 16 CTAs, 32 streams over 2000 cells 37 us unsplit (256 CTAs) and 43 us
     // over 2.  More rows than slots: two parts even out streams of different
-    // length (64 streams of 500 to 8100 cells: 154 to 146 us).  A part is at
+    // length (64 streams of 698 to 8100 cells: 154 to 146 us).  A part is at
     // least a warp step for each warp.
-    // Where a cluster of 16 is all there is and few of them, eight warps a CTA.
+    // Where a cluster of 16 is all there is and few of them, eight warps a CTA
+    // (one stream over 32701 cells in 4 bits: 37 to 35 us, two 55 to 47; heads
+    // of 128 in 8 bits have room for one stage a warp then).
     const int64_t slots = 3 * (int64_t) sm_count;
     const int     warps = p.few && 2 * base * 16 <= slots && reach >= kStep * 8 * 16 ? 8 : 4;
     const int64_t most  = std::min<int64_t>(16, std::max<int64_t>(1, reach / (kStep * warps)));

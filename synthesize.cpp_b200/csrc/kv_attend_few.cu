@@ -25,9 +25,9 @@
 // steps, because the tensor cores cut their sums off where fp32 addition
 // rounds.
 //
-// 64 streams of 500 to 8100 positions (keys in 8 bits, values in 4; 519 MB):
-// 145 us, 3.6 TB/s; its copies alone take 85 us.  It is bound by instructions
-// with fixed latencies: a step of 32 cells is about 825, at 2.6 warps a
+// 64 streams of 698 to 8100 positions (keys in 8 bits, values in 4; 519 MB):
+// 142 us, 3.7 TB/s; its copies alone take 85 us.  It is bound by instructions
+// with fixed latencies: a step of 32 cells is about 850, at 2.6 warps a
 // scheduler or fewer.  A stream alone (32701 positions, Q4_0): 34 us, because
 // its 128 CTAs do not fill the SMs.
 #include "kv_attend.cuh"

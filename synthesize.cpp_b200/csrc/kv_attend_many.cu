@@ -28,9 +28,10 @@
 // operand tiles up to three: copies, conversion, MMAs and weights of
 // neighbouring tiles overlap.
 //
-// A 4096-token prompt over 4-bit caches, 16 heads of 128 in F32: 267 us (257
+// A 4096-token prompt over 4-bit caches, 16 heads of 128 in F32: 271 us (254
 // TFLOP/s of attention, which take three times as many fp16 ones; on mma.sync
-// 797 us).  What bounds it is the chain of a tile: it takes the row warps
+// 797 us).  Ragged bf16 prompts (5761 rows after up to 901, Q8_0): 257 us, with
+// weights of one part 244.  What bounds it is the chain of a tile: it takes the row warps
 // about 2300 cycles, the code warps 1900 and the tensor cores 1536.
 #include "kv_attend.cuh"
 

@@ -4,7 +4,7 @@
 // a key row's chunk of the block, or two neighbouring chunks of a value row.
 // The largest magnitude is folded over the four lanes by shuffles, each lane
 // rounds its own values, and its codes are one or two aligned stores.  It is
-// bound by the rounding, about ten operations a value: 12 prompts (11400 rows
+// bound by the rounding, about ten operations a value: 12 prompts (12187 rows
 // of 8 heads of 128) take 34 us, 3.4 TB/s (with four values a lane 41 us: half
 // of the work was addresses and folds).
 // Reading back: eight lanes a block, so that a lane's four floats are next to
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_write_kernel(const KvRowsArgs 
                 scale   = !(top <= 3.40282347e38f) ? 0x7e00u : __half_as_ushort(__float2half_rn(d));
             } else {
                 const float top = block_amax<4, 8>(v, part);
-                const float d   = __fmul_rn(top, 0.00787401574803149606f);  // RN(1/127)
+                const float d   = __fmul_rn(top, 0.00787401574803149606f);  // RN(1/127): the header's definition
                 const float id  = d != 0.0f ? __frcp_rn(d) : 0.0f;
                 // own > top: a value before the block's last NaN, which the fold of magnitudes leaves out
                 if (__all_sync(0xffffffffu, top >= 1e-30f && top <= 1e30f && own <= top)) {

@@ -11,7 +11,8 @@ rows ``starts[i]:starts[i+1]`` at positions ``pos[i]``, ``pos[i] + 1``, ... of s
 each run is one row, without ``slots`` run i is slot i; ``max_len`` bounds the runs' lengths (left out, the number of rows does; a close bound
 makes a faster call).  ``pos``, ``slots`` and ``starts`` are int32 CUDA tensors.  Work is enqueued on torch's current
 stream of the cache's device, whichever device is current; a failure raises B200Q8Error, and what only the device can see
-(a position outside the cache) is reported by ``q8.device_status``.
+(a position outside the cache) is reported by ``q8.device_status``.  Rows that no run names are left alone: where a call
+allocates its result, they hold whatever the memory held.  Nothing here is recorded for gradients.
 """
 from __future__ import annotations
 
